@@ -18,7 +18,6 @@ code is a sign bit and an index into 0 .5 1 1.5 2 3 4 6; scale byte b stands for
 """
 from __future__ import annotations
 
-import functools
 import math
 import sys
 from pathlib import Path
@@ -437,7 +436,6 @@ def _run_plain(st):
     return st["out"]
 
 
-@functools.lru_cache(maxsize=None)
 def _package():
     pkg = str(Path(__file__).resolve().parent.parent / "flash-dllm_amd")
     if pkg not in sys.path:
