@@ -2,7 +2,8 @@
 //
 // A head's row of 128 channels is four groups of 32 channels, each 4-bit floats (a sign and one of
 // 0 .5 1 1.5 2 3 4 6) times a power of two: the number format of CDNA4's scaled MFMAs and of its
-// 4-bit converters, so the attention feeds K to the matrix cores as stored. 4.25 bits per value.
+// 4-bit converters: the importance feeds K to the matrix cores as stored, the attention converts two values
+// an instruction to bf16, exactly. 4.25 bits per value.
 //
 // Cell = 16 consecutive slots of one K/V head, kCellBytes bytes; the cells of a slot group's heads lie
 // side by side: cache[slot / 16][kv_head][kCellBytes]. In a cell, slot s (0..15):

@@ -7,13 +7,15 @@
 //    under the Flash-Verify mask.
 //
 // Per 64-key block and operand of 16 query rows
-//    S^T = K Q^T   v_mfma_scale_f32_16x16x128_f8f6f4, K as stored (4-bit codes, a scale per 32
-//                  channels and key), Q as two 8-bit parts: q = hi + lo up to 2^-22 of the row's
-//                  largest element (a bf16 has 8 significant bits, an e4m3 has 4). The same matrix
-//                  rate as bf16, and K needs no conversion. Within a group the instruction drops what
-//                  lies 2^-13 below the largest product: of a logit far less than what rounding P
-//                  to bf16 costs.
-//    O^T = V^T P^T v_mfma_f32_16x16x32_bf16, V converted (exact in bf16), P rounded to bf16 as the bf16
+//    S^T = K Q^T   v_mfma_f32_16x16x32_bf16, K converted in registers (exact in bf16: two significant bits
+//                  times a power of two), so a logit is a 32-bit sum of exact products. The scaled MFMA
+//                  takes K as stored and Q as two 8-bit parts at the same matrix rate, but aligns the
+//                  products of a 32-channel group to the largest and drops what lies 2^-13 below it: with
+//                  one channel of a query far above the others, outputs were 8 times as far off as
+//                  the rounding of P allows. The conversions cost 0-3% of a call (8 x 1024 rows and
+//                  keys, whose issue slots are full: 163 -> 172 us; one token 11.1 -> 10.7, for Q needs
+//                  no parts).
+//    O^T = V^T P^T v_mfma_f32_16x16x32_bf16, V converted alike, P rounded to bf16 as the bf16
 //                  cache's attention does; the rows' sums of P are one more row of V^T, all ones, so
 //                  they are of the rounded P and cost no vector instructions.
 // Keys sit so that nothing moves between lanes. Of a block's 64 keys, MFMA row mm of the t-th K operand
@@ -100,50 +102,26 @@ __device__ __forceinline__ int q_scale(float top) {
 }
 __device__ __forceinline__ float exp2i(int biased) { return __uint_as_float(uint32_t(biased) << 23); }
 
-// Rounds the four values of x to e4m3, returns their bytes and leaves 32 times the remainders in x.
-__device__ __forceinline__ int fp8_part(float (&x)[4]) {
-  int w = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
-  w = __builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], w, true);
-  x[0] = 32.f * (x[0] - __builtin_amdgcn_cvt_f32_fp8(w, 0));
-  x[1] = 32.f * (x[1] - __builtin_amdgcn_cvt_f32_fp8(w, 1));
-  x[2] = 32.f * (x[2] - __builtin_amdgcn_cvt_f32_fp8(w, 2));
-  x[3] = 32.f * (x[3] - __builtin_amdgcn_cvt_f32_fp8(w, 3));
-  return w;
-}
-
-// The 128 channels of a query as the B operand: the scaled MFMA's lane group g holds channels
-// 16 g .. 16 g + 15 and 64 + 16 g .. (4-bit operands: 32 g .. 32 g + 31).
+// The 128 channels of a query as four B operands: lane group g's share of operand x is channels 32 g + 8 x ..,
+// word x of the 32 channels that the lane holds of a key. A query with a NaN or an infinity is NaN as a
+// whole: its logits, which may all be the same infinity, are then never taken for keys left out.
 struct QFrag {
-  i32x8 hi, lo;
-  int scale;  // byte 0: of hi, byte 1: of lo
+  u32x4 x[4];
 };
 
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+
 __device__ __forceinline__ QFrag load_q(const uint16_t* row, int g, bool valid) {
-  float x[32];
-  float top = 0.f;
-#pragma unroll
-  for (int h = 0; h < 4; ++h) {
-    const u32x4 w = valid ? ld16(row + 16 * g + 64 * (h >> 1) + 8 * (h & 1)) : u32x4{0, 0, 0, 0};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      x[8 * h + 2 * j] = __uint_as_float(w[j] << 16);
-      x[8 * h + 2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < 32; ++j) top = fmaxf(top, fabsf(x[j]));
-  const int e = q_scale(xmax(top));
-  const float down = exp2i(254 - e);
   QFrag f;
+  u16x2 top = {0, 0};
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    float y[4];
+  for (int x = 0; x < 4; ++x) {
+    f.x[x] = valid ? ld16(row + 32 * g + 8 * x) : u32x4{0, 0, 0, 0};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) y[i] = x[4 * j + i] * down;
-    f.hi[j] = fp8_part(y);
-    f.lo[j] = fp8_part(y);
+    for (int j = 0; j < 4; ++j)
+      top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, f.x[x][j] & 0x7fff7fffu));
   }
-  f.scale = e | ((e - 5) << 8);
+  if (top[0] >= 0x7f80 || top[1] >= 0x7f80) f.x[0][0] = ~0u;
   return f;
 }
 
@@ -156,15 +134,6 @@ struct Block {
   u32x4 v[4];
   u32x4 vs;
 };
-
-// One K operand (byte t of ks: its scales) times one part of Q (byte `part` of scale), added to s.
-template <int t, int part>
-__device__ __forceinline__ f32x4 mfma_kq(u32x4 k, uint32_t ks, i32x8 q, int scale, f32x4 s) {
-  const i32x8 a = {static_cast<int>(k.x), static_cast<int>(k.y), static_cast<int>(k.z),
-                   static_cast<int>(k.w), 0, 0, 0, 0};
-  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, q, s, 4, 0, t, static_cast<int>(ks),
-                                                          part, scale);
-}
 
 // The state of R x 16 query rows: lane (c, g) holds query c's reference maximum (log2 units), the sum of
 // its probabilities (in every element of l), and O^T: element e of o[.][i] is O^T row 4 g + e of the
@@ -245,18 +214,28 @@ __device__ __forceinline__ f32x4 add_sums(f32x4 l, u32x4 p) {
   return mfma16(as_bf16x8(ones), as_bf16x8(p), l);
 }
 
-// Logits of a cache block's K operands (byte t of ks: operand t's scales).
-__device__ __forceinline__ void logits(const u32x4 (&k)[4], uint32_t ks, const QFrag& q,
-                                       f32x4 (&s)[4]) {
-  const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-  s[0] = mfma_kq<0, 0>(k[0], ks, q.hi, q.scale, zero);
-  s[1] = mfma_kq<1, 0>(k[1], ks, q.hi, q.scale, zero);
-  s[2] = mfma_kq<2, 0>(k[2], ks, q.hi, q.scale, zero);
-  s[3] = mfma_kq<3, 0>(k[3], ks, q.hi, q.scale, zero);
-  s[0] = mfma_kq<0, 1>(k[0], ks, q.lo, q.scale, s[0]);
-  s[1] = mfma_kq<1, 1>(k[1], ks, q.lo, q.scale, s[1]);
-  s[2] = mfma_kq<2, 1>(k[2], ks, q.lo, q.scale, s[2]);
-  s[3] = mfma_kq<3, 1>(k[3], ks, q.lo, q.scale, s[3]);
+// Logits of a cache block's K operands (byte t of ks: operand t's scales), converted a word at a time for all
+// R operands of queries: four sums side by side to each, of exact products in 32 bits.
+template <int R>
+__device__ __forceinline__ void logits(const u32x4 (&k)[4], uint32_t ks, const QFrag (&q)[R],
+                                       f32x4 (&s)[R][4]) {
+  float scale[4];
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    scale[t] = __uint_as_float((ks >> (8 * t) & 255u) << 23);
+#pragma unroll
+    for (int r = 0; r < R; ++r) s[r][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+#pragma unroll
+  for (int x = 0; x < 4; ++x)
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const uint32_t w = k[t][x];
+      const u32x4 a = {kv4_bf16x2<0>(w, scale[t]), kv4_bf16x2<1>(w, scale[t]),
+                       kv4_bf16x2<2>(w, scale[t]), kv4_bf16x2<3>(w, scale[t])};
+#pragma unroll
+      for (int r = 0; r < R; ++r) s[r][t] = mfma16(as_bf16x8(a), as_bf16x8(q[r].x[x]), s[r][t]);
+    }
 }
 
 // Keys that do not count (bit 4 e + t of ok clear) leave the softmax.
@@ -679,8 +658,7 @@ __global__ __launch_bounds__(64 * kWaves, R == 1 ? 3 : 2) void kv4_wave_kernel(K
     float scale[R];
     f32x4 s[R][4];
     u32x4 p[R][2];
-#pragma unroll
-    for (int r = 0; r < R; ++r) logits(blk.k, blk.ks, q[r], s[r]);
+    logits<R>(blk.k, blk.ks, q, s);
     if constexpr (kImp)
       if (imp)
         importance_block(a, blk.k, blk.ks, frags, kvh, lane,
@@ -828,11 +806,11 @@ __device__ __forceinline__ uint32_t seen_keys(const Kv4Args& a, int64_t vb, int 
   return bits & below(n_in, at);
 }
 
-// The verify block's own 64 keys from ib * 64 on: K (bf16) in kbuf, 16-byte chunk x * 4 + g of key 4 c + t at
+// The verify block's own 64 keys from ib * 64 on: K (bf16) in kbuf, channels 32 g + 8 x .. of key 4 c + t at
 // ((t * 16 + 4 x + g) * 16 + c) * 16, V in vbuf as above with its NaNs and infinities left out (`odd`: there
 // are some): 0 times them would reach rows that do not see the key.
 template <int R>
-__device__ __forceinline__ void own_keys(const Kv4Args& a, Rows<R>& st, const int64_t (&orow)[R],
+__device__ __forceinline__ void own_keys(const Kv4Args& a, Rows<R>& st, const QFrag (&q)[R],
                                          const int (&qi)[R], int64_t q0, int n_in, int64_t vb,
                                          int kvh, int T, int S, int ib, bool odd,
                                          const uint8_t* kbuf, const uint8_t* vbuf, int c, int g) {
@@ -842,10 +820,6 @@ __device__ __forceinline__ void own_keys(const Kv4Args& a, Rows<R>& st, const in
   uint32_t seen[R];  // bit 4 e + t: the lane's query sees key j0 + 16 g + 4 e + t
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    u32x4 q[4];
-#pragma unroll
-    for (int x = 0; x < 4; ++x)
-      q[x] = ld16(a.q + max(orow[r], int64_t(0)) * kHeadDim + 32 * x + 8 * g);
     seen[r] = seen_keys(a, vb, T, S, qi[r], n_in, j0 + 16 * g);
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
@@ -853,7 +827,7 @@ __device__ __forceinline__ void own_keys(const Kv4Args& a, Rows<R>& st, const in
 #pragma unroll
       for (int x = 0; x < 4; ++x)
         s[r][t] = mfma16(as_bf16x8(ld16(kbuf + ((t * 16 + 4 * x + g) * 16 + c) * 16)),
-                         as_bf16x8(q[x]), s[r][t]);
+                         as_bf16x8(q[r].x[x]), s[r][t]);
     }
     hide(s[r], seen[r]);
   }
@@ -891,8 +865,7 @@ __device__ __forceinline__ void own_keys(const Kv4Args& a, Rows<R>& st, const in
 
 // Bound by issue and power: 8 x 1024 rows and keys of 32 heads in 150-165 us (0.9 PFLOP/s; MFMAs busy 0.37 of
 // the cycles, LDS 0.21, vector instructions 0.4, at 1.8-2 GHz). Neither fewer vector instructions (no
-// maximum per block: 168), nor wavefront priorities (159-166), nor Q in 6-bit parts, which halves the time
-// of its MFMAs (153 for 161, and 2^-13 of a group's largest element lost), help enough. Verify over 16 x
+// maximum per block: 168) nor wavefront priorities (159-166) help enough. Verify over 16 x
 // 64 rows and 946-978 gathered keys of 32 heads: 46 us, of which 11 for the own keys and the start; 32 rows
 // to a wavefront with the blocks halved between two pairs of wavefronts: 45, and 15.8 for one sequence of
 // 264 keys instead of 14.9.
@@ -1074,12 +1047,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv4_tile_kernel(Kv4Args a) {
       if (row >= 0 && row < a.n_q_rows) orow[r] = row * a.heads + kvh * G + m % G;
     }
   }
-  auto load_queries = [&]() {
 #pragma unroll
-    for (int r = 0; r < R; ++r)
-      q[r] = load_q(a.q + max(orow[r], int64_t(0)) * kHeadDim, g, orow[r] >= 0);
-  };
-  if (!kVerify || kOwnAhead) load_queries();
+  for (int r = 0; r < R; ++r)
+    q[r] = load_q(a.q + max(orow[r], int64_t(0)) * kHeadDim, g, orow[r] >= 0);
   const bool idle = m0 + wave * R * 16 >= t.rows * G;  // no rows: the wavefront only moves blocks
 
   const bool imp = kImp && t.n_imp > 0 && m0 == 0;
@@ -1101,7 +1071,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv4_tile_kernel(Kv4Args a) {
       for (int x = 0; x < 4; ++x) {
         const int kk = 64 * kWaves * x + tid;
         const int n = 4 * (kk >> 2 & 15) + (kk >> 8), cc = (kk & 3) + 4 * (kk >> 6 & 3);
-        st16(smem + kVBuf + ((n & 3) * 256 + cc * 16 + (n >> 2)) * 16, own_k[x]);
+        st16(smem + kVBuf + ((n & 3) * 256 + (4 * (cc & 3) + (cc >> 2)) * 16 + (n >> 2)) * 16, own_k[x]);
         const int vn = kk >> 4, w = kk & 15;
         u32x4 v = own_v[x];
         if (kBlockKeys * ib + vn >= t.rows) v = u32x4{0, 0, 0, 0};
@@ -1116,10 +1086,9 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv4_tile_kernel(Kv4Args a) {
       odd = __syncthreads_or(odd);
       if (kOwnAhead && ib + 1 < own_hi) own_load(ib + 1);
       if (!idle)
-        own_keys<R>(a, st, orow, qi, q0, t.rows, item, kvh, T, S, ib, odd, smem + kVBuf, smem, c, g);
+        own_keys<R>(a, st, q, qi, q0, t.rows, item, kvh, T, S, ib, odd, smem + kVBuf, smem, c, g);
       __syncthreads();
     }
-    if (!kOwnAhead) load_queries();
   }
   for (int lo = b_lo; lo < b_hi; lo += kVerify ? kChunk : b_hi - b_lo) {
     const int hi = kVerify ? min(lo + kChunk, b_hi) : b_hi;
@@ -1169,8 +1138,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void kv4_tile_kernel(Kv4Args a) {
           read_k(k, ks, b);
           const uint32_t ok = keys_ok(b, g);
           const bool edge = __any(ok != 0xffffu);
-#pragma unroll
-          for (int r = 0; r < R; ++r) logits(k, ks, q[r], s[r]);
+          logits<R>(k, ks, q, s);
           if (edge)
 #pragma unroll
             for (int r = 0; r < R; ++r) hide(s[r], ok);
