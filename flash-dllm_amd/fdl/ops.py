@@ -767,7 +767,14 @@ def _kv4_parts(plan: AttnPlan, first: int, count: int, rows: int, group: int, kv
     6000 keys of 8 heads 140 -> 22. Few equal tokens that divide the compute units get one workgroup each
     (16000 keys of 8 heads 10.7 us, with three to a unit 13.2; 8 tokens over 8000 19.6, 21.4); uneven ones
     as many as fit, whose last parts even out (8 over 1000 to 32000: 34 to 49 us, with one each 36 to
-    49)."""
+    49).
+
+    Tiles of more than 32 rows that fill the compute units are cut only where the longest stream at least
+    halves: then those far above the mean set the time (64 rows of 32 heads over 65501 keys beside seven
+    over 768: 1092 us uncut, 165 in 15 parts; 96 rows, four tiles over 32000 beside four over 768 733, 338). Equal ones
+    are left alone, and so are those of the mean length or below while they have up to 32 blocks, whose
+    partial rows cost more than they bring (two over 1536 beside six over 768: 33 us uncut, 38 in 3 parts;
+    one over 8000 beside eleven over 1000: 143 uncut, 63 in parts of 20 blocks, 51 in parts of 26)."""
     rows, total, most = _kv4_tiles(plan, first, count, rows)
     rows = max(rows, 1)
     m = rows * group
@@ -776,18 +783,22 @@ def _kv4_parts(plan: AttnPlan, first: int, count: int, rows: int, group: int, kv
                                 (64, 1, 2) if m <= 64 else (128, 1, 2))
     wgs = kv_heads * -(-m // wg_rows)
     # half a part of every tile's last one is empty on average
-    slots = max(per_cu * cus - count * wgs // 2, per_cu * cus // 4)
+    full = streams == 1 and count * wgs >= cus
+    cut = total // max(most, 1) if full else count  # (about as many tiles are far above the mean)
+    slots = max(per_cu * cus - cut * wgs // 2, per_cu * cus // 4)
     equal, one_each = total == count * most, cus - cus % max(count * wgs, 1)
     if equal and m <= 16 and 4 * count * wgs <= cus and 8 * one_each >= 7 * cus:
         slots = one_each
     per = max(-(-total * wgs // slots), streams)
     per = -(-per // streams) * streams
+    if full:
+        per = max(per, min(-(-total // count), 32))
     limit = _kv4_most_parts(count, rows, kv_heads, group, wgs)
-    if most - per < 6 * streams or (streams == 1 and count * wgs >= cus) or limit < 2:
+    if most - per < 6 * streams or (full and 2 * per > most) or limit < 2:
         return rows, 1, max(most, 1)
     parts = min(-(-most // per), limit)
-    if equal:
-        per = -(-most // parts)
+    # fewer parts than asked for are longer ones, not a last one with all the rest
+    per = -(-most // parts) if equal else max(per, -(-most // parts))
     return rows, parts, per
 
 
