@@ -6,9 +6,9 @@
 //        k'[c + 64] = k[c + 64] cos[c + 64] + k[c] sin[c + 64]
 //  * fdl_kv4_read: the rows of slots as bf16, exactly what the codes stand for.
 //
-// The rotation runs in 64 bits and is rounded to 32 once: a bf16 times a float is exact in 64 bits, so
-// the rotated value is correctly rounded and the codes do not depend on how a compiler orders or fuses
-// the arithmetic (a value next to the border of two codes would otherwise flip a whole step).
+// The rotation runs in 64 bits and is rounded once, K to 32 bits, Q to bf16: a bf16 times a float is exact in
+// 64 bits, so the rotated value is correctly rounded and the codes do not depend on how a compiler orders
+// or fuses the arithmetic (a value next to the border of two codes would otherwise flip a whole step).
 #include "fdl_host.h"
 #include "fdl_kv4.h"
 
@@ -62,6 +62,16 @@ __device__ __forceinline__ float group_top(const float (&x)[8]) {
   return fmaxf(top, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(top), 0x4E, 0xF, 0xF, false)));
 }
 
+// A float half way between two bf16 values: rounded from a double it says no more on which side the double was.
+__device__ __forceinline__ bool half_way(float f) { return __float_as_uint(f) << 16 == 0x80000000u; }
+
+// Such a float, moved by a bit to the double's side, so that its rounding to bf16 is the double's.
+__device__ __forceinline__ float to_side(float f, double d) {
+  const double to = fabs(d), at = fabs(static_cast<double>(f));
+  const uint32_t b = __float_as_uint(f);
+  return !half_way(f) || to == at ? f : __uint_as_float(to > at ? b + 1 : b - 1);
+}
+
 // One unit of 8 lanes per (row, head of K, V or Q), the heads of a row side by side: whole 64-byte runs of
 // every input row, and a lane's two words of codes need no other lane. Bound by memory: 7919 rows with Q of
 // 32 heads and K and V of 8, rotated, in 35 us (200 MB, 5.7 TB/s, part of it in the Infinity Cache); by
@@ -103,11 +113,23 @@ __global__ __launch_bounds__(kThreads) void kv4_append_kernel(AppendArgs a) {
     load8(sp + 64, s1);
     load8(cp, c0);
     load8(cp + 64, c1);
+    bool again = false;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const double x = lo[j], y = hi[j];
       lo[j] = static_cast<float>(x * c0[j] - y * s0[j]);
       hi[j] = static_cast<float>(y * c1[j] + x * s1[j]);
+      again = again || half_way(lo[j]) || half_way(hi[j]);
+    }
+    if (what == kQ && again) {  // one lane in 4000: a second look (for every value: 2 of 48 us of 7919 rows)
+      float x[8], y[8];
+      unpack8(src, x);
+      unpack8(src + 64, y);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        lo[j] = to_side(lo[j], double(x[j]) * c0[j] - double(y[j]) * s0[j]);
+        hi[j] = to_side(hi[j], double(y[j]) * c1[j] + double(x[j]) * s1[j]);
+      }
     }
   }
   if (what == kQ) {
