@@ -48,9 +48,12 @@ def _regions(cache: torch.Tensor):
 
 
 def store_rows(cache: torch.Tensor, slot: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> None:
-    """Quantises K and V rows [n, n_kv_heads * 128] into cache slots slot [n] (distinct)."""
+    """Quantises K and V rows [n, n_kv_heads * 128] into cache slots slot [n] (distinct); rows with a slot
+    outside the cache (padding: -1) are skipped."""
     kr, vr, ks, vs = _regions(cache)
     heads = cache.shape[1]
+    inside = (slot >= 0) & (slot < 16 * cache.shape[0])
+    slot, k, v = slot[inside], k[inside], v[inside]
     cell, s = slot // 16, slot % 16
     codes, scales = quantize_rows(k.reshape(-1, heads, HEAD_DIM))
     kr[cell, :, s] = codes
@@ -68,8 +71,11 @@ def _decode(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
 
 
 def load_rows(cache: torch.Tensor, slot: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
-    """K and V rows [n, n_kv_heads * 128] float32 of cache slots."""
+    """K and V rows [n, n_kv_heads * 128] float32 of cache slots; zeros for a slot outside the cache."""
     kr, vr, ks, vs = _regions(cache)
+    outside = (slot < 0) | (slot >= 16 * cache.shape[0])
+    slot = torch.where(outside, 0, slot)
     cell, s = slot // 16, slot % 16
-    return (_decode(kr[cell, :, s], ks[cell, :, :, s]),
+    rows = (_decode(kr[cell, :, s], ks[cell, :, :, s]),
             _decode(vr[cell, :, s // 4, :, s % 4].flatten(-2), vs[cell, :, :, s]))
+    return tuple(x.masked_fill(outside[:, None], 0.0) for x in rows)
