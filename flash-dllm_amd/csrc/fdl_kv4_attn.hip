@@ -1244,8 +1244,8 @@ int check_common(const char* fn, const void* q, const void* cache, const void* o
               (long long)n_slots);
   FDL_REQUIRE(n_q_rows >= 1 && n_q_rows < (int64_t(1) << 31), FDL_ERR_SHAPE,
               "%s: n_q_rows = %lld out of range", fn, (long long)n_q_rows);
-  FDL_REQUIRE(softmax_scale > 0.f && softmax_scale <= 3.4e38f, FDL_ERR_SHAPE,
-              "%s: softmax_scale must be positive and finite", fn);
+  FDL_REQUIRE(softmax_scale > 0.f && softmax_scale <= 2.3e38f, FDL_ERR_SHAPE,
+              "%s: softmax_scale must be positive and at most 2.3e38 (log2(e) times it is finite)", fn);
   const void* const ptrs[] = {q, cache, out};
   const char* const names[] = {"q", "cache", "out"};
   for (int i = 0; i < 3; ++i) {

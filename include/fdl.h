@@ -507,7 +507,7 @@ int fdl_kv4_read(const void* cache, int64_t n_slots, int64_t n_kv_heads, int64_t
  *   imp_mode FDL_IMP_NONE or FDL_IMP_RAW_LOGIT; imp_part fp32 [n_heads][n_slots] as for
  *            fdl_block_attention (at most 16 query heads to a K/V head); NaN for a head whose
  *            importance rows hold a NaN or an infinity
- *   softmax_scale > 0
+ *   softmax_scale > 0, at most 2.3e38
  *   n_parts, part_blocks: each tile's 64-key blocks in up to n_parts (1..FDL_KV4_MAX_PARTS) runs of
  *            part_blocks blocks, the last one with the rest, each in workgroups of its own; a second
  *            kernel merges them. workspace fp32 of n_parts * n_work * tile_rows * n_heads *
@@ -532,7 +532,7 @@ int fdl_kv4_attention(const void* q, const void* cache, int64_t n_q_rows, int64_
  *   q, out bf16 [n_q_rows][n_heads * 128]; k_blk, v_blk bf16 [n_q_rows][n_kv_heads * 128] (the block's own
  *   rows as keys stay bf16: they are not in the cache yet). A NaN or infinity in v_blk reaches only
  *   the rows that see its key; a row that sees no key is zero. Keys whose slot lies outside the
- *   cache are left out. softmax_scale > 0.
+ *   cache are left out. softmax_scale > 0, at most 2.3e38.
  *   n_parts, part_blocks: as for fdl_kv4_attention, over a block's runs of 64 own keys, then of 64 cache
  *   keys; workspace fp32 of n_parts * n_vblocks * block_rows * n_heads * FDL_KV4_PART_FLOATS floats for
  *   n_parts > 1.

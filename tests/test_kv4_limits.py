@@ -1,7 +1,8 @@
-"""The 4-bit cache without a GPU: slots outside the cache in the plain form."""
+"""The 4-bit cache without a GPU: slots outside the cache in the plain form, and the largest softmax scales."""
+import pytest
 import torch
 
-from fdl import kv4, ops
+from fdl import kv4, lib, ops
 
 
 def test_plain_rows_outside_the_cache_are_skipped_and_read_as_zeros():
@@ -19,3 +20,14 @@ def test_plain_rows_outside_the_cache_are_skipped_and_read_as_zeros():
     before = cache.clone()
     kv4.store_rows(cache, torch.tensor([-1, 32, -16, 99, 40]), k, v)
     assert torch.equal(cache, before)
+
+
+@pytest.mark.parametrize("scale", [2.4e38, 3.4e38])
+def test_softmax_scales_whose_base_2_form_is_infinite_are_refused(scale):
+    p = 0x10000  # never read: the calls end before a launch
+    with pytest.raises(lib.FdlError, match="softmax_scale"):
+        lib.call("fdl_kv4_attention", p, p, 4, 64, 8, 2, 128, p, 1, 2, 5, p, 1, p, 4, 4, scale, p, 0, None,
+                 1, 1, None, 0, None)
+    with pytest.raises(lib.FdlError, match="softmax_scale"):
+        lib.call("fdl_kv4_verify_attention", p, p, p, p, 64, 64, 4, 2, 128, p, 8, p, 1, None, p, 64, scale, p,
+                 1, 1, None, 0, None)
