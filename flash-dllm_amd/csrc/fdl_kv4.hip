@@ -74,7 +74,7 @@ __device__ __forceinline__ float to_side(float f, double d) {
 
 // One unit of 8 lanes per (row, head of K, V or Q), the heads of a row side by side: whole 64-byte runs of
 // every input row, and a lane's two words of codes need no other lane. Bound by memory: 7919 rows with Q of
-// 32 heads and K and V of 8, rotated, in 35 us (200 MB, 5.7 TB/s, part of it in the Infinity Cache); by
+// 32 heads and K and V of 8, rotated, in 35.5 us (179 MB, 5.0 TB/s); by
 // the launch for few rows (8: 3.4 us).
 __global__ __launch_bounds__(kThreads) void kv4_append_kernel(AppendArgs a) {
   const int64_t unit = (int64_t(blockIdx.x) * kThreads + threadIdx.x) / kUnitLanes;
@@ -158,7 +158,7 @@ __global__ __launch_bounds__(kThreads) void kv4_append_kernel(AppendArgs a) {
   }
 }
 
-// As above: 8 lanes per (row, head of K or V). A row without a slot in the cache reads as zeros. 4096 rows
+// As above: 8 lanes per (row, head of K or V). A row without a slot in the cache reads as zeros. 8192 rows
 // of 8 heads: 9 us.
 __global__ __launch_bounds__(kThreads) void kv4_read_kernel(
     const uint8_t* __restrict__ cache, int64_t n_slots, int kv_heads,

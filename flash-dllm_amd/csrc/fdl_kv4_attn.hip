@@ -12,9 +12,9 @@
 //                  takes K as stored and Q as two 8-bit parts at the same matrix rate, but aligns the
 //                  products of a 32-channel group to the largest and drops what lies 2^-13 below it: with
 //                  one channel of a query far above the others, outputs were 8 times as far off as
-//                  the rounding of P allows. The conversions cost 0-3% of a call (8 x 1024 rows and
-//                  keys, whose issue slots are full: 163 -> 172 us; one token 11.1 -> 10.7, for Q needs
-//                  no parts).
+//                  the rounding of P allows. The conversions cost up to 3.4% (8 x 1024 rows and keys,
+//                  whose issue slots are full: 153 -> 158 us; one token over 2011 keys 9.4 -> 9.0, since
+//                  Q needs no parts).
 //    O^T = V^T P^T v_mfma_f32_16x16x32_bf16, V converted alike, P rounded to bf16 as the bf16
 //                  cache's attention does; the rows' sums of P are one more row of V^T, all ones, so
 //                  they are of the rounded P and cost no vector instructions.
@@ -568,10 +568,10 @@ __device__ __forceinline__ float inverse(float l) { return l == 0.f ? 0.f : 1.f 
 
 constexpr int kWaves = 4;
 
-// Bound by memory where there are many keys: 24 tokens of 32 heads over 368403 keys of 8 heads in 84 us (401
-// MB, 4.8 TB/s; 0.2 of the wavefronts' cycles issue vector work), 32 rows of 32 heads over 65501 keys in 62
-// (4.7 TB/s), 70 with the importance, whose 4 MFMAs and 20 additions a block no longer hide; by the chain
-// of loads at its start and by the merge for few (2011 keys: 6.7 us + 3 of merging).
+// Bound by memory where there are many keys: 24 tokens of 32 heads over 368403 keys of 8 heads in 85 us (401
+// MB, 4.7 TB/s; 0.22 of the wavefronts' cycles issue vector work), 32 rows of 32 heads over 65501 keys in 63
+// (4.6 TB/s), 67-71 with the importance, whose 4 MFMAs and 20 additions a block no longer hide; by the chain
+// of loads at its start and by the merge for few (2011 keys: 6.4 us + 3 of merging).
 //
 // R x 16 rows per workgroup. Lane (c, g) ends with channels 32 g + 8 e + i of query c in o[.][i][e]: the
 // i-th V^T operand's row m is channel 8 m + i, i.e. word m of a key's codes.
@@ -863,17 +863,17 @@ __device__ __forceinline__ void own_keys(const Kv4Args& a, Rows<R>& st, const QF
     }
 }
 
-// Bound by issue and power: 8 x 1024 rows and keys of 32 heads in 150-165 us (0.9 PFLOP/s; MFMAs busy 0.37 of
-// the cycles, LDS 0.21, vector instructions 0.4, at 1.8-2 GHz). Neither fewer vector instructions (no
-// maximum per block: 168) nor wavefront priorities (159-166) help enough. Verify over 16 x
-// 64 rows and 946-978 gathered keys of 32 heads: 46 us, of which 11 for the own keys and the start; 32 rows
-// to a wavefront with the blocks halved between two pairs of wavefronts: 45, and 15.8 for one sequence of
-// 264 keys instead of 14.9.
+// Bound by issue and power: 8 x 1024 rows and keys of 32 heads in 158 us (0.87 PFLOP/s; MFMAs busy 0.35 of
+// the cycles, LDS 0.20, vector instructions 0.3 of the wavefronts'). Verify over 16 x 64 rows and 946-978
+// gathered keys of 32 heads: 45.5 us, of which 11 for the own keys and the start. Tried with K on the scaled
+// MFMA, where the first took 150-165 us in one run or another: no maximum per block 168, wavefront
+// priorities 159-166; 32 rows to a wavefront with the blocks halved between two pairs of wavefronts 45 for
+// 47 us of the second, and 15.8 for 14.9 with one sequence of 264 keys.
 //
 // 16 R rows to a wavefront. A wavefront brings its cell of each block; kAhead blocks are in registers, on
 // their way, and two are in LDS. Four wavefronts of up to 32 rows, so that workgroups of different phases
 // share a compute unit: eight in one workgroup took 163 us on 8 x 1024 rows and keys of 32 heads where
-// four take 156, also with half of them a phase behind the others (172).
+// four took 156 (K on the scaled MFMA), also with half of them a phase behind the others (172).
 template <int R, int kAhead, bool kImp, bool kVerify>
 __global__ __launch_bounds__(64 * kWaves, 2) void kv4_tile_kernel(Kv4Args a) {
   static_assert(kAhead == 2 || kAhead == 4, "the buffers alternate, the ring is a power of two");

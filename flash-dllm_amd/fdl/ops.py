@@ -771,10 +771,10 @@ def _kv4_parts(plan: AttnPlan, first: int, count: int, rows: int, group: int, kv
 
     Tiles of more than 32 rows that fill the compute units are cut only where the longest stream at least
     halves: then those far above the mean set the time (64 rows of 32 heads over 65501 keys beside seven
-    over 768: 1092 us uncut, 165 in 15 parts; 96 rows, four tiles over 32000 beside four over 768 733, 338). Equal ones
-    are left alone, and so are those of the mean length or below while they have up to 32 blocks, whose
-    partial rows cost more than they bring (two over 1536 beside six over 768: 33 us uncut, 38 in 3 parts;
-    one over 8000 beside eleven over 1000: 143 uncut, 63 in parts of 20 blocks, 51 in parts of 26)."""
+    over 768: 1092 us uncut, 165 in 15 parts; 96 rows, four tiles over 32000 beside four over 768: 733,
+    338). Equal ones are left alone, and so are those of the mean length or below while they have up to 32
+    blocks, whose partial rows cost more than they bring (two over 1536 beside six over 768: 33 us uncut,
+    38 in 3 parts; one over 8000 beside eleven over 1000: 143 uncut, 63 in parts of 20 blocks, 51 of 26)."""
     rows, total, most = _kv4_tiles(plan, first, count, rows)
     rows = max(rows, 1)
     m = rows * group
