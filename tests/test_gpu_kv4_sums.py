@@ -118,3 +118,23 @@ def test_infinite_queries_are_nan(rows, keys):
     assert got[odd].isnan().all()
     o, tol = _expected(torch.where(odd[..., None], 0.0, q.double().view(rows, heads, 128)), k, v)
     plain.close(got[~odd], o[~odd], tol[~odd])
+
+
+@pytest.mark.parametrize("lowest", [0, 2, 120])
+@pytest.mark.parametrize("rows,keys", [(1, 70), (20, 70), (40, 130), (100, 70)])
+def test_tiny_keys_and_huge_queries(lowest, rows, keys):
+    """Groups at the smallest scales, whose values are below the smallest normal bf16, times queries as large as
+    that makes ordinary logits."""
+    rng = np.random.default_rng(rows + lowest)
+    heads, n_slots = 2, 160
+    cache = plain.random_cache(rng, n_slots, heads)
+    cache[..., 2048:2112] = rng.integers(lowest, lowest + 2, cache[..., 2048:2112].shape)
+    cache[..., 2112:] = 127
+    q = torch.from_numpy(0.3 * rng.standard_normal((rows, heads * 128)) * 2.0 ** (126 - lowest)).to(BF16)
+    plan = make_plan([SeqRows(batch=0, k_end=keys, rows=np.arange(rows))],
+                     np.arange(n_slots // 32, dtype=np.int32)[None], 5, device=DEV)
+    out = torch.zeros(q.shape, dtype=BF16, device=DEV)
+    ops.kv4_attention(q.to(DEV), _dev(cache), plan, out, heads, SCALE)
+    k, v = (torch.from_numpy(x) for x in plain.get(cache, np.arange(keys)))
+    o, tol = _expected(q.double().view(rows, heads, 128), k, v)
+    plain.close(out.double().cpu().view(rows, heads, 128), o, tol)
